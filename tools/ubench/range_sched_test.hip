@@ -2,7 +2,7 @@
 // waves, "processing" a plane = the wave counts itself into counts[(col * nplanes + x) * 4 + wave] and sleeps for a
 // pseudo-random, column-dependent time (skewed work: some columns cost 4x the others, so a lot is stolen).  At the end every
 // (column, plane, wave) must have been counted exactly once.
-// build: hipcc --offload-arch=gfx950 -O3 -mllvm -amdgpu-atomic-optimizer-strategy=None tools/ubench/range_sched_test.hip -o tools/ubench/range_sched_test
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -mllvm -amdgpu-atomic-optimizer-strategy=None tools/ubench/range_sched_test.hip -o tools/ubench/range_sched_test
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,5 +1,5 @@
 // Microbenchmark: how fast can gfx950 stream a 512 MiB fp32 field through "compare -> sign word"?
-// Variants differ in load width and batching.  Build: hipcc --offload-arch=gfx950 -O3 stream_variants.hip
+// Variants differ in load width and batching.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops stream_variants.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

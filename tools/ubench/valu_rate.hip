@@ -2,7 +2,7 @@
 // waves resident on the SIMD?  (Decides whether a kernel's SQ_INSTS_VALU x 4 cycles or x 2 cycles is its issue floor.)
 // Each wave runs a long unrolled stream of independent instructions of one kind over 8 registers; blocks of 256 x W
 // threads put W waves on every SIMD of a CU, one block per CU.  Reports cycles per instruction per SIMD from s_memtime.
-// build: hipcc --offload-arch=gfx950 -O3 tools/ubench/valu_rate.hip -o tools/ubench/valu_rate
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench/valu_rate.hip -o tools/ubench/valu_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

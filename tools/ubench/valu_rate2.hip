@@ -1,6 +1,6 @@
 // Per-instruction issue cost on one SIMD with 4 resident waves (the regime of the face and streaming kernels): which
 // of the integer / select / shift instructions run at the 2-cycle rate and which at the 4-cycle one?
-// build: hipcc --offload-arch=gfx950 -O3 tools/ubench/valu_rate2.hip -o tools/ubench/valu_rate2
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench/valu_rate2.hip -o tools/ubench/valu_rate2
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
