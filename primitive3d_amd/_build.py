@@ -50,8 +50,8 @@ def _write_stamp(out: Path, deps, extra=""):
     out.with_name(out.name + ".stamp").write_text(_digest(deps, extra) + "\n")
 
 
-# k_fused's plane claims are `if (lane == 0) old = atomic add`, consumed one plane later: LLVM's atomic optimizer would
-# rewrite that into a wave reduction that reads the result (and waits for it) right behind the atomic
+# k_fused's output cursors are `if (lane == 0) got = atomic add`, consumed a batch of vertices later: LLVM's atomic optimizer
+# would rewrite that into a wave reduction that reads the result (and waits for it) right behind the atomic
 CAPI_EXTRA_FLAGS = ["-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
 
 

@@ -1,11 +1,11 @@
 """Properties of the COMPILED kernels that their speed leans on and that the source cannot promise (hipcc cross-compiles
 without a GPU, so this runs in the CPU suite):
 
-  * the cursor atomic of k_fused is ONE scalar-memory atomic per wave-plane (`s_atomic_add ... glc`, counted by lgkmcnt):
-    a vector atomic in its place would queue its result behind the wave's vector stores and plane loads again;
-  * its destination register is written ASYNCHRONOUSLY (the compiler does not know): nothing may read, copy or spill it
-    between the atomic and the hand-written `s_waitcnt lgkmcnt(0)` that hands it over;
-  * no other atomic lives in that kernel;
+  * the cursor atomic of k_fused is ONE returning vector atomic per wave-plane, and its result is awaited by a COUNTED
+    wait that leaves the NU plane loads issued behind it in flight (a wait for everything would pay the memory latency and
+    the arithmetic of every plane one after the other);
+  * beside it and the spill area's cursor no other atomic lives in that kernel;
+  * no kernel writes memory through the scalar unit: what it does there is load;
   * no k_fused / k_faces / k_face_count_walk variant uses scratch memory.
 """
 import re
@@ -28,8 +28,7 @@ def device_asm(tmp_path_factory):
     spec = importlib.util.spec_from_file_location("p3d_build", ROOT / "primitive3d_amd" / "_build.py")
     build = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(build)
-    cmd = [HIPCC if Path(HIPCC).exists() else "hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",
-           *build.CAPI_EXTRA_FLAGS, "-S",
+    cmd = [HIPCC if Path(HIPCC).exists() else "hipcc", *build.HIP_FLAGS, *build.CAPI_EXTRA_FLAGS, "-S",
            "--cuda-device-only", str(ROOT / "primitive3d_amd" / "csrc" / "p3d_mc.hip"), "-o", str(out)]
     subprocess.run(cmd, check=True, capture_output=True, timeout=900)
     return out.read_text()
@@ -45,69 +44,59 @@ def _kernels(asm, name):
     return out
 
 
-_WAIT = re.compile(r"#ASMSTART\s*\n\s*s_waitcnt lgkmcnt\(0\)\s*\n\s*;;#ASMEND")
+def _instructions(body):
+    """Instruction lines of a kernel's text, without comments, labels and directives."""
+    lines = (ln.split(";")[0].strip() for ln in body.split("\n"))
+    return [ln for ln in lines if ln and not ln.endswith(":") and not ln.startswith(".")]
 
 
-def _sregs(text):
-    """Scalar registers a line of assembly mentions: s7 -> {7}, s[16:17] -> {16, 17}."""
+def _vregs(text):
+    """Vector registers a line of assembly mentions: v7 -> {7}, v[16:17] -> {16, 17}."""
     regs = set()
-    for a, b in re.findall(r"\bs\[(\d+):(\d+)\]", text):
+    for a, b in re.findall(r"\bv\[(\d+):(\d+)\]", text):
         regs.update(range(int(a), int(b) + 1))
-    regs.update(int(r) for r in re.findall(r"\bs(\d+)\b", text))
+    regs.update(int(r) for r in re.findall(r"\bv(\d+)\b", text))
     return regs
 
 
-def test_cursor_atomic_is_scalar(device_asm):
+def test_one_vector_atomic_per_wave_plane(device_asm):
     kernels = _kernels(device_asm, "k_fused")
-    assert len(kernels) == 8   # 4 tile geometries x 2 sample types (the round-4 DYN variants left in round 5)
+    assert len(kernels) == 8   # 4 tile geometries x 2 sample types
     for name, body in kernels.items():
+        atomics = [ins for ins in _instructions(body) if "atomic" in ins.split()[0]]
         # one cursor atomic per half of the unrolled plane loop, and behind each the spill area's (region-layout mode, the rare
-        # wave-plane that does not fit: awaited inside its own asm statement)
-        assert body.count("s_atomic_add ") == 4, name
-        assert len(re.findall(r"s_atomic_add s\d+, s\[\d+:\d+\], 0x0 glc\n\s*s_waitcnt lgkmcnt\(0\)", body)) == 2, name
-        assert "s_atomic_add_x2" not in body and "buffer_atomic" not in body, name
-        assert "global_atomic" not in body, name
-        # the results are awaited by the hand-written scalar-counter wait, right in front of the slot computation
-        assert len(_WAIT.findall(body)) >= 2, name
+        # wave-plane that does not fit): word 8 of a cursor line
+        assert len(atomics) == 4, (name, atomics)
+        assert all(re.fullmatch(r"global_atomic_add v\d+, v\d+, v\d+, s\[\d+:\d+\]( offset:64)? sc0", ins) for ins in atomics), (name, atomics)
+        assert sum("offset:64" in ins for ins in atomics) == 2, (name, atomics)
 
 
-def test_async_atomic_results_are_left_alone(device_asm):
-    """`got` is an SGPR written by a scalar atomic that is still in flight when its asm statement ends.  Until the
-    hand-written lgkmcnt(0) wait that hands it over nothing may read, copy or spill it -- a copy there reads the stale value
-    (round 4: a second scalar atomic made the compiler move the operand to another register pair in front of the wait;
-    round 6: a second hand-written wait on the same variable made it copy the register right in front of the real one).
-    Checked on the text, block by block (block placement is the compiler's, and the register is reused for other values in
-    blocks that run BEFORE the atomic but stand behind it in the file, so a scan in file order says nothing):
-      A. from the atomic to the end of its basic block no instruction mentions its destination;
-      B. in the basic block of every hand-written wait, between the block's label and the wait, no instruction READS a
-         register an atomic of the kernel writes.
-    What this cannot see -- a copy in a block in between -- shows as wrong vertex ids: tests/test_gpu_parity.py compares
-    them on every path (the counting pass's records alone included, since the round-6 case was masked by a later pass)."""
+def test_cursor_result_is_awaited_by_a_count(device_asm):
+    """Between a cursor atomic and the first reader of its result stand exactly the NU row loads of the prefetched plane and
+    a wait that leaves those NU in flight; nothing in between reads, copies or overwrites the register, and no wait in
+    between is stricter."""
     for name, body in _kernels(device_asm, "k_fused").items():
-        lines = body.split("\n")
-        atomics = [(i, _sregs(m.group(1))) for i, ln in enumerate(lines) for m in [re.match(r"\s*s_atomic_add (s\d+),", ln)] if m]
-        assert len(atomics) >= 2, name
-        dests = set().union(*(d for _, d in atomics))
-        for i, dest in atomics:
-            j = i + 1
-            if "s_waitcnt lgkmcnt(0)" in lines[j]:
-                continue   # (awaited inside its own asm statement: the spill area's atomic)
-            while j < len(lines) and not re.match(r"\s*\.LBB\w+:", lines[j]):
-                if "s_waitcnt lgkmcnt(0)" in lines[j] and "ASMSTART" in lines[j - 1]:
-                    break
-                assert not (dest & _sregs(lines[j].split(";")[0])), (name, "A", i, lines[i].strip(), j, lines[j].strip())
-                j += 1
-        waits = [j for j, ln in enumerate(lines) if "s_waitcnt lgkmcnt(0)" in ln and "ASMSTART" in lines[j - 1]]
-        assert len(waits) >= 2, name
-        for w in waits:
-            j = w - 2   # (w - 1 is the ASMSTART line)
-            while j >= 0 and not re.match(r"\s*\.LBB\w+:", lines[j]):
-                ins = lines[j].split(";")[0].strip()
-                m = re.match(r"(\S+)\s+([^,]+),(.*)", ins)
-                if m and not ins.startswith(("s_cbranch", "s_branch")):
-                    sources = _sregs(m.group(3))   # everything behind the first operand: what the instruction reads
-                    assert not (dests & sources), (name, "B", w, j, lines[j].strip())
-                j -= 1
+        nc, ry = map(int, re.search(r"k_fusedI\w*?Li(\d+)ELi(\d+)E", name).groups())
+        nu = (ry + 1) * nc
+        ins = _instructions(body)
+        cursors = [i for i, ln in enumerate(ins) if ln.startswith("global_atomic_add") and "offset:64" not in ln]
+        assert len(cursors) == 2, name
+        for i in cursors:
+            dest = int(re.match(r"global_atomic_add v(\d+),", ins[i]).group(1))
+            use = next(j for j in range(i + 1, len(ins)) if dest in _vregs(ins[j]))
+            assert re.fullmatch(r"v_readfirstlane_b32 s\d+, v%d" % dest, ins[use]), (name, ins[i], ins[use])
+            between = ins[i + 1:use]
+            loads = sum(ln.startswith(("buffer_load", "global_load", "flat_load")) for ln in between)
+            others = [ln for ln in between if re.match(r"(buffer|global|flat|scratch)_(store|atomic)", ln)]
+            assert loads == nu and not others, (name, loads, others)
+            waits = [int(m.group(1)) for ln in between for m in [re.search(r"\bvmcnt\((\d+)\)", ln)] if m]
+            assert waits and min(waits) == waits[-1] == nu, (name, waits)
+
+
+def test_scalar_unit_only_loads(device_asm):
+    for ins in _instructions(device_asm):
+        op = ins.split()[0]
+        assert not (op.startswith("s_") and ("atomic" in op or "store" in op)), ins
 
 
 def test_no_scratch_in_the_benchmarked_variants(device_asm):
