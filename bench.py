@@ -745,7 +745,8 @@ def main():
 
     elapsed = t1 - t0
     if world > 1:
-        t = torch.tensor([elapsed], dtype=torch.float64, device=dev)
+        comm_dev = dev if dist.get_backend() == "nccl" else "cpu"   # (gloo, the dry run's transport, moves host memory only)
+        t = torch.tensor([elapsed], dtype=torch.float64, device=comm_dev)
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
         elapsed = float(t.item())
     nvox_total = rx * ry * rz * batch
@@ -755,7 +756,7 @@ def main():
     out_v, out_f = out
     nv, nf = int(out_v.shape[0]), int(out_f.shape[0])
     if world > 1:
-        cnt = torch.tensor([nv, nf], dtype=torch.int64, device=dev)
+        cnt = torch.tensor([nv, nf], dtype=torch.int64, device=comm_dev)
         dist.all_reduce(cnt)
         nv, nf = int(cnt[0]), int(cnt[1])
 

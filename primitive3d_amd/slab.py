@@ -239,6 +239,27 @@ class SlabResult:
         return iter((self.vertices, self.faces))
 
 
+class _HostStagedShift:
+    """A neighbour exchange of device tensors over gloo: gloo moves host memory only (its collectives on device tensors have
+    hung when several ranks shared one GPU), so the sent plane is copied to the host before the transfer is posted and the
+    received one to the device when it has arrived.  Both copies are synchronous and in the order of the current stream."""
+
+    def __init__(self, dist, send, dst, recv, src):
+        self.recv = recv
+        self.host_send = send.cpu().contiguous() if send is not None else None
+        self.host_recv = torch.empty(recv.shape, dtype=recv.dtype) if recv is not None else None
+        ops = [dist.P2POp(dist.isend, self.host_send, dst)] if send is not None else []
+        if recv is not None:
+            ops.append(dist.P2POp(dist.irecv, self.host_recv, src))
+        self.works = dist.batch_isend_irecv(ops) if ops else []
+
+    def wait(self):
+        for w in self.works:
+            w.wait()
+        if self.recv is not None:
+            self.recv.copy_(self.host_recv)
+
+
 class SlabExtractor:
     def __init__(self, shape: Sequence[int], rank: int, world: int, device, dtype=torch.float32, backend=None,
                  hold_planes: int = 2):
@@ -367,7 +388,13 @@ class SlabExtractor:
         lower = [0.0, 0.0, 0.0] if lower is None else lower
         upper = [rx, ry, rz] if upper is None else upper
 
+        # RCCL collectives are ordered after the work already enqueued on the current stream.  gloo (CPU transport, used
+        # by the tests and the single-GPU dry run) gets host copies of what it exchanges.
+        gloo_on_gpu = self.grid.is_cuda and dist.get_backend() == "gloo"
+
         def shift_to_prev(send, recv):  # rank r sends to r-1, receives from r+1: nearest-neighbour only
+            if gloo_on_gpu:
+                return [_HostStagedShift(dist, send, self.rank - 1, recv, self.rank + 1)]
             ops = []
             if send is not None:
                 ops.append(dist.P2POp(dist.isend, send, self.rank - 1))
@@ -375,18 +402,9 @@ class SlabExtractor:
                 ops.append(dist.P2POp(dist.irecv, recv, self.rank + 1))
             return dist.batch_isend_irecv(ops) if ops else []
 
-        # RCCL collectives are ordered after the work already enqueued on the current stream.  gloo (CPU transport, used
-        # by the tests and the single-GPU dry run) reads device tensors without that ordering: synchronise for it.
-        gloo_on_gpu = self.grid.is_cuda and dist.get_backend() == "gloo"
-
-        def pre_comm():
-            if gloo_on_gpu:
-                torch.cuda.synchronize()
-
         # the halo plane travels while the interior planes are already being streamed
         self._marks = []
         self._mark("start")
-        pre_comm()
         works = shift_to_prev(self.halo_send_buffer(), self.halo_recv_buffer())
         self.phase_interior(thresh, lower, upper)
         self._mark("interior planes streamed")
@@ -405,12 +423,17 @@ class SlabExtractor:
             rank_counts = torch.empty((self.world, 3), dtype=torch.int64, device=self.grid.device)
             send_buf = self.records_send_buffer()  # (kept referenced until the transfer has completed)
             self._mark("last planes streamed + record export")
-            pre_comm()
             # ASYNCHRONOUS: the plain form makes the current stream wait for the collective right here (torch's non-async
             # collectives end in work.wait()), i.e. the face count below would start only when the slowest rank's count had
             # arrived -- the all-gather's latency and the ranks' skew on every rank's critical path.  Waited for in front
             # of the face launch, the only consumer (round 6: it had been the plain form since round 3).
-            gathered = dist.all_gather_into_tensor(rank_counts.view(-1), be.header_words(), async_op=True)
+            if gloo_on_gpu:
+                host_counts = torch.empty(rank_counts.shape, dtype=rank_counts.dtype)
+                dist.all_gather_into_tensor(host_counts.view(-1), be.header_words().cpu())
+                rank_counts.copy_(host_counts)
+                gathered = None
+            else:
+                gathered = dist.all_gather_into_tensor(rank_counts.view(-1), be.header_words(), async_op=True)
             self._mark("all-gather of vertex counts")
             rec_works = shift_to_prev(send_buf, self.records_recv_buffer())
             be.launch_finalize(defer_totals=True)   # (from the second call on: the faces follow with a capacity guess)
@@ -452,10 +475,10 @@ class SlabExtractor:
                 raise OverflowError(self.ID_OVERFLOW % self.rank)
             return SlabResult(self._verts, faces, rank=self.rank, rank_counts=rank_counts, check=check)
         nv, nf = self.phase_extract(thresh, lower, upper)
-        mine = torch.tensor([nv, nf, 1 if self.id_overflow() else 0], dtype=torch.int64, device=self.grid.device)
+        mine = torch.tensor([nv, nf, 1 if self.id_overflow() else 0], dtype=torch.int64,
+                            device="cpu" if gloo_on_gpu else self.grid.device)
         allc = [torch.empty_like(mine) for _ in range(self.world)]
         send_buf = self.records_send_buffer()
-        pre_comm()
         dist.all_gather(allc, mine)
         gathered = torch.stack(allc).cpu()
         counts = [(int(c[0]), int(c[1])) for c in gathered]
