@@ -161,11 +161,13 @@ def build_rc(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_all(force: bool = False, verbose: bool = False):
-    a = build_capi(force, verbose)
-    build_capi(force, verbose, dev=True)
-    d = build_rc(force, verbose)     # (the pybind adapter links it)
-    b = build_pybind(force, verbose)
-    c = build_mt(force, verbose)
+    from concurrent.futures import ThreadPoolExecutor
+    with ThreadPoolExecutor(4) as pool:   # (each step is a compiler process of its own)
+        a, _, c, d = [f.result() for f in (pool.submit(build_capi, force, verbose),
+                                           pool.submit(build_capi, force, verbose, dev=True),
+                                           pool.submit(build_mt, force, verbose),
+                                           pool.submit(build_rc, force, verbose))]
+    b = build_pybind(force, verbose)      # (links the first and the last of them)
     return a, b, c, d
 
 

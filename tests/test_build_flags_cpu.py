@@ -37,3 +37,18 @@ def test_no_packed_fp32(build, step, tmp_path, monkeypatch):
     asm = out.read_text()
     assert ".amdhsa_kernel" in asm
     assert not re.findall(r"\bv_pk_(?:add|mul|fma)_f32\b", asm)
+
+
+def test_build_compiles_where_libraries_are_there(built, tmp_path, monkeypatch):
+    """__graft_entry__.build() is the check that the sources compile: a library that is already there does not answer it."""
+    import __graft_entry__
+    mod = __graft_entry__.load_build_module()
+    commands = []
+    monkeypatch.setattr(mod.subprocess, "check_call", commands.append)
+    monkeypatch.setattr(mod, "_write_stamp", lambda *a: None)
+    monkeypatch.setattr(mod, "_stale", lambda *a: False)
+    monkeypatch.setattr(mod, "PKG", tmp_path)   # (nothing is written beside the package)
+    monkeypatch.setattr(__graft_entry__, "load_build_module", lambda: mod)
+    __graft_entry__.build()
+    outs = sorted(Path(c[c.index("-o") + 1]).relative_to(mod.PKG).as_posix() for c in commands if "-o" in c)
+    assert outs == sorted(["libp3dmc.so", "dev/libp3dmc.so", "libp3dmt.so", "libp3drc.so", mod.pybind_path().name])
